@@ -41,3 +41,21 @@ def test_index_names_files_that_exist():
                 if at.is_dir() and not list(at.glob(word)):
                     missing.append(f"{folder}/{word}")
     assert not missing, missing
+
+
+def test_scene20_probe_runs_default_builds_only():
+    # dbg20.py compares frames of the 10k-sphere scene with the oracle under environment variants given as "label|ENV=V".
+    # A 6-wave build of that scene faulted the GPU, so scripts run the probe on the default build alone ("label|"): no
+    # forced register budget, no code compiled out, no other library
+    bad = []
+    for name, text in _sources():
+        if not name.endswith(".sh"):
+            continue
+        for line in text.splitlines():
+            if line.lstrip().startswith("#") or "dbg20.py" not in line:
+                continue
+            before, after = line.split("dbg20.py", 1)
+            variants = re.findall(r'"([^"|]*)\|([^"]*)"', after)
+            if "RT_HIP_LIB" in before or not variants or any(env for _, env in variants):
+                bad.append(f"{name}: {line.strip()[:90]}")
+    assert not bad, bad
