@@ -18,8 +18,12 @@ INC       := -Iinclude -I$(CSRC)
 
 # No FP contraction anywhere on the path: parity with the oracle is bit-exact.
 HOST_FLAGS := -O2 -std=c++17 -fPIC -ffp-contract=off -fno-fast-math -Wall -Wextra
+# No packed f32 instructions: some operand forms of v_pk_{add,mul,fma}_f32 have given wrong results on the MI355X now and
+# then, without an error, and the compiler forms them from plain float code (the host pass warns that it does not know
+# the feature).
+NO_PACKED_F32 := -Xclang -target-feature -Xclang -packed-fp32-ops
 HIP_FLAGS  := -O3 -std=c++17 -fPIC --offload-arch=$(ARCH) -ffp-contract=off -fno-fast-math \
-              -fhip-fp32-correctly-rounded-divide-sqrt -fno-gpu-rdc -fno-slp-vectorize -Wall
+              -fhip-fp32-correctly-rounded-divide-sqrt -fno-gpu-rdc -fno-slp-vectorize $(NO_PACKED_F32) -Wall
 ORACLE_FLAGS := -O2 -std=c11 -fPIC -ffp-contract=off -fno-fast-math -fopenmp -Wall -Wextra
 
 HOST_SRC := $(CSRC)/host/rt_host.cpp $(CSRC)/host/image_load.cpp $(CSRC)/host/image_jpeg.cpp \

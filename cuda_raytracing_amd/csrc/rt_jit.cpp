@@ -266,15 +266,18 @@ bool jit_source(const SceneImage &img, int variant, uint32_t max_visits, bool fo
 }
 
 // The complete hipRTC option vector.  Same numerics flags as the offline build.  SLP vectorisation is
-// off: on this code it packs scalar f32 pairs into v_pk_* with extra moves, turns the planar inside-test
-// into a <4 x i1> reduction, and its longer live ranges spill ~100 SGPRs (measured: -10% instructions,
+// off: on this code it pairs scalar f32 operations with extra moves, turns the planar inside-test
+// into a <4 x i1> reduction, and its longer live ranges spill ~100 SGPRs (measured with packed instructions: -10% instructions,
 // 86 -> 71 VGPRs on scene 0; measured again in round 1: +30 % frame time).  RT_JIT_OPTS appends options
 // (A/B experiments); hipRTC keeps the FIRST of two conflicting flags, so it cannot override these.
 // The on-disk cache key hashes this whole vector (build_module): bit-exact parity rests on these flags.
 std::vector<std::string> jit_options(const std::string &arch, const std::vector<std::string> &extra) {
   std::vector<std::string> o = {"--offload-arch=" + arch, "-O3", "-std=c++17", "-ffp-contract=off", "-fno-fast-math",
                                 "-fhip-fp32-correctly-rounded-divide-sqrt"};
-  // RT_JIT_SLP=1 (A/B): let the SLP vectoriser pack f32 pairs into v_pk_* (off by default, above)
+  // No packed f32 instructions, as in the offline build: some operand forms of v_pk_{add,mul,fma}_f32 have given wrong
+  // results on the MI355X now and then, without an error.
+  for (const char *f : {"-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"}) o.push_back(f);
+  // RT_JIT_SLP=1 (A/B): let the SLP vectoriser form f32 pairs (off by default, above); they are computed one by one
   if (const char *e = std::getenv("RT_JIT_SLP"); !(e && e[0] == '1')) o.push_back("-fno-slp-vectorize");
   // Loops are unrolled only where the source asks (#pragma unroll): ROCm 7.2's LLVM 22 otherwise also unrolls the
   // colour-stack unwind and the rejection loops of the scene-specialised kernels (+11 % static VALU instructions, scene 0

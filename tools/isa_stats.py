@@ -38,7 +38,8 @@ def main():
     out.mkdir(parents=True, exist_ok=True)
     (out / "k.hip").write_text("#include <hip/hip_runtime.h>\n" + buf.value.decode())
     cmd = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fno-fast-math",
-           "-fhip-fp32-correctly-rounded-divide-sqrt", "-fno-slp-vectorize", *a.flags.split(),
+           "-fhip-fp32-correctly-rounded-divide-sqrt", "-fno-slp-vectorize",
+           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", *a.flags.split(),
            f"-I{REPO / 'cuda_raytracing_amd/csrc/device'}", "--cuda-device-only", "-c", "k.hip", "-o", "k.o",
            "-save-temps"]
     r = subprocess.run(cmd, cwd=out, capture_output=True, text=True)

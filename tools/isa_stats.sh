@@ -15,7 +15,7 @@ open(sys.argv[2] + "/k.hip", "w").write("#include <hip/hip_runtime.h>\n" + src)
 PY
 cd "$out"
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -fno-fast-math \
-  -fhip-fp32-correctly-rounded-divide-sqrt -fno-slp-vectorize $ISA_FLAGS -I"$repo/cuda_raytracing_amd/csrc/device" --cuda-device-only \
+  -fhip-fp32-correctly-rounded-divide-sqrt -fno-slp-vectorize -Xclang -target-feature -Xclang -packed-fp32-ops $ISA_FLAGS -I"$repo/cuda_raytracing_amd/csrc/device" --cuda-device-only \
   -c k.hip -o k.o -save-temps 2>&1 | grep -E "error" || true
 s=$(ls k-hip-amdgcn-amd-amdhsa-gfx950.s)
 awk '/^rt_static_render:/,/s_endpgm/' "$s" > k0.s

@@ -1,5 +1,6 @@
 // valu_peak.hip — measured VALU issue rates of one MI355X, for the roofline peak of bench.py.
-//   hipcc --offload-arch=gfx950 -O3 -fno-slp-vectorize tools/valu_peak.hip -o tools/valu_peak && tools/valu_peak
+//   P='-Xclang -target-feature -Xclang -packed-fp32-ops'   # no packed f32, as in every HIP build here
+//   hipcc --offload-arch=gfx950 -O3 -fno-slp-vectorize $P tools/valu_peak.hip -o tools/valu_peak && tools/valu_peak
 // Each thread runs 16 independent chains of one instruction kind, 8 waves per SIMD; prints the
 // lane-instructions per second of each kind and the ratio to 256 CU x 4 SIMD x 32 lanes/clk x 2.4 GHz.
 #include <hip/hip_runtime.h>
@@ -20,13 +21,6 @@ __global__ __launch_bounds__(256) void op_kernel(float *out, float a, float b) {
       else if (OP == 1) x[c] = x[c] + a;                       // v_add_f32
       else if (OP == 2) x[c] = x[c] * a;                       // v_mul_f32
       else if (OP == 4) x[c] = (c & 1) ? x[c] * a : x[c] + b;  // mul/add mix
-    }
-    if (OP == 5) {                                              // v_pk_fma_f32: 2 f32 fmas per lane
-      typedef float f2 __attribute__((ext_vector_type(2)));
-      f2 *y = reinterpret_cast<f2 *>(x);
-      const f2 a2 = {a, a}, b2 = {b, b};
-#pragma unroll
-      for (int c = 0; c < kChains / 2; ++c) y[c] = __builtin_elementwise_fma(y[c], a2, b2);
     }
   }
   float s = 0.0f;
@@ -65,11 +59,11 @@ int main() {
   const int cus = prop.multiProcessorCount;
   const int blocks = cus * 8;   // 8 blocks x 4 waves per CU = 8 waves per SIMD
   const double spec = static_cast<double>(cus) * 4 * 32 * 2.4e9;
-  const double r[5] = {rate<0>(out, blocks, 1), rate<1>(out, blocks, 1), rate<2>(out, blocks, 1),
-                       rate<4>(out, blocks, 1), rate<5>(out, blocks, 1)};
-  const char *names[5] = {"v_fma_f32", "v_add_f32", "v_mul_f32", "v_mul_f32/v_add_f32", "v_pk_fma_f32 (2 fma/lane)"};
+  const double r[4] = {rate<0>(out, blocks, 1), rate<1>(out, blocks, 1), rate<2>(out, blocks, 1),
+                       rate<4>(out, blocks, 1)};
+  const char *names[4] = {"v_fma_f32", "v_add_f32", "v_mul_f32", "v_mul_f32/v_add_f32"};
   std::printf("{\"cus\": %d, \"clock_mhz\": %d, \"spec_lane_ops_per_s\": %.4e, \"rates\": {", cus, prop.clockRate / 1000, spec);
-  for (int k = 0; k < 5; ++k)
+  for (int k = 0; k < 4; ++k)
     std::printf("%s\"%s\": {\"lane_ops_per_s\": %.4e, \"fraction_of_spec\": %.4f}", k ? ", " : "", names[k], r[k], r[k] / spec);
   std::printf("}}\n");
   (void)hipFree(out);
